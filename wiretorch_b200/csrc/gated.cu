@@ -20,8 +20,8 @@
 // registers and their maps joined over a block or over a cluster's shared memory, reads them
 // once, but took 50 instructions an element and waited at its barriers: 32 x 10,000 x 256 bf16
 // 0.22 ms forward and 0.46 backward against 0.15 and 0.21, 1 x 131,072 x 64 fp32 0.20 and 0.21
-// against 0.05 and 0.06. A product of decays above 1 over a part (up to T / 2 steps) has to stay
-// in float's range; where it does not, a state that enters it as 0 is still right.
+// against 0.05 and 0.06. The product of the decays over a stretch of time has to stay in float's
+// range; where growing ones leave it, a state that enters the stretch as 0 is still right.
 //
 // The backward pass recomputes h inside a segment of kSteps steps from the float state that
 // enters it: the forward's own output for float, states it saved on the way for 16-bit types
@@ -130,9 +130,16 @@ __device__ __forceinline__ float keeps() {
     return SIG ? __int_as_float(0x7f800000) : 1.0f;
 }
 
-// s -> A s + H. A state of 0 takes no part where a product of growing decays overflowed.
+// s -> A s + H. A state of 0 takes no part where a product of growing decays overflowed; A is not a
+// number where one of them was not finite.
 __device__ __forceinline__ float follow(float A, float H, float s) {
     return s == 0.0f && !isnan(A) ? H : __fmaf_rn(A, s, H);
+}
+
+// The product of two parts' decays: infinity stands for one that overflowed, which a decay of 0 ends.
+__device__ __forceinline__ float product(float A, float a) {
+    const float p = A * a;
+    return isnan(p) && !isnan(A) && !isnan(a) ? 0.0f : p;
 }
 
 // The threads of a trial's columns, and the columns of a thread: adjacent ones where rows allow
@@ -339,10 +346,12 @@ struct Maps {
     __device__ __forceinline__ float *H(int b, int p, int N) const { return A(b, p, N) + N; }
 };
 
-// Each part's map, FORWARD of h' = f h + u, else of adj' = f (adj + dh). The part is walked
-// against the direction of the walk behind it (each step's term enters by the product of the decays
-// that follow it), which then begins with what was read last and is still in L2. `operand` is x or dh.
-// 32 x 10,000 x 256 bf16: 57 us, 5.8 TB/s, instructions issued in 60-70% of the cycles.
+// Each part's map, FORWARD of h' = f h + u, else of adj' = f (adj + dh); `operand` is x or dh. The part is
+// walked in its own order from a state of 0, so that H is what the walk behind it would come to: adding each
+// step's term times the product of the decays that follow makes 0 times infinity of a term of 0
+// where those grow past float's range (and walking against time for it, to begin the next walk with what
+// is still in L2, was worth at most 1%: 208 against 210 us of the backward pass of 32 x 10,000 x 256
+// bf16). There 57 us, 5.8 TB/s, instructions issued in 60-70% of the cycles.
 template <typename E, bool SIG, bool WIDE, bool CUTS, bool FORWARD, typename Args>
 __global__ void __launch_bounds__(block_of(WIDE)) maps_kernel(const Args s, const void *operand, long long o_b, long long o_t, const Maps maps) {
     extern __shared__ __align__(16) unsigned char dynamic[];
@@ -356,7 +365,7 @@ __global__ void __launch_bounds__(block_of(WIDE)) maps_kernel(const Args s, cons
     const E *a = static_cast<const E *>(s.a) + at.b * s.a_b, *o = static_cast<const E *>(operand) + at.b * o_b;
     const uint8_t *starts = CUTS ? s.starts + (long long)at.b * s.T : nullptr;
     const int end = min(at.hi, at.len), tiles = end > at.lo ? (end - at.lo + kSteps - 1) / kSteps : 0;
-    auto first = [&](int i) { return at.lo + (FORWARD ? tiles - 1 - i : i) * kSteps; };
+    auto first = [&](int i) { return at.lo + (FORWARD ? i : tiles - 1 - i) * kSteps; };
     auto fetch = [&](int i) {
         const int t0 = first(i);
         const E *row[2] = {a + t0 * s.a_t, o + t0 * o_t};
@@ -375,8 +384,8 @@ __global__ void __launch_bounds__(block_of(WIDE)) maps_kernel(const Args s, cons
         copies_end_group();
     }
     next_may_start();
-    float A[V] = {1.0f, 1.0f, 1.0f, 1.0f}, H[V] = {}, most[V] = {};  // most: of the decays' size
-    bool cut = false;  // a start was met: steps beyond it have no part
+    float A[V] = {1.0f, 1.0f, 1.0f, 1.0f}, H[V] = {}, most[V] = {}, least[V] = {1.0f, 1.0f, 1.0f, 1.0f};
+    bool cut = false;  // a start was met: what enters the part is dropped
     const int rounds = kMeet ? __reduce_max_sync(live, tiles) : tiles;
     for (int i = 0; i < rounds; i++) {
         if (kMeet) __syncwarp(live);  // the other thread has read the slots that are filled next
@@ -389,8 +398,8 @@ __global__ void __launch_bounds__(block_of(WIDE)) maps_kernel(const Args s, cons
         const unsigned bits = CUTS ? starts_of(starts + first(i), end - first(i)) : 0;
 #pragma unroll
         for (int m = 0; m < kSteps; m++) {
-            const int k = FORWARD ? kSteps - 1 - m : m;
-            const bool start = CUTS && (bits >> k & 1), on = !cut;
+            const int k = FORWARD ? m : kSteps - 1 - m;
+            const bool start = CUTS && (bits >> k & 1);
             float f[V], u[V];
             stage[i % kHold].get(0, k, view, keeps<E, SIG>(), f);
             stage[i % kHold].get(1, k, view, 0.0f, u);
@@ -398,23 +407,29 @@ __global__ void __launch_bounds__(block_of(WIDE)) maps_kernel(const Args s, cons
             for (int j = 0; j < V; j++) {
                 float g;
                 gate<E, SIG>(f[j], f[j], g);
-                if (!SIG) most[j] = fmaxf(most[j], on && !start ? fabsf(f[j]) : 0.0f);
+                if (!SIG) {
+                    most[j] = fmaxf(most[j], fabsf(f[j]));
+                    least[j] = fminf(least[j], fabsf(f[j]));
+                }
                 if (FORWARD) {
                     if (SIG) u[j] *= g;
-                    H[j] = on ? __fmaf_rn(A[j], u[j], H[j]) : H[j];
-                    A[j] *= f[j];
+                    H[j] = start ? u[j] : __fmaf_rn(f[j], H[j], u[j]);
                 } else {
-                    A[j] *= f[j];
-                    H[j] = on && !start ? __fmaf_rn(A[j], u[j], H[j]) : H[j];
+                    H[j] = start ? 0.0f : f[j] * (H[j] + u[j]);
                 }
+                A[j] *= f[j];
             }
             cut |= start;
         }
     }
 #pragma unroll
     for (int j = 0; j < V; j++) {
-        // an infinite decay makes a state of 0 not a number, an overflowed product of finite ones does not
-        if (!SIG && isinf(most[j])) A[j] = CUDART_NAN_F;
+        if (!SIG) {
+            // an infinite decay makes a state of 0 not a number; of finite ones a single 0 makes the product
+            // 0, though it may have overflowed
+            if (isinf(most[j])) A[j] = CUDART_NAN_F;
+            else if (least[j] == 0.0f) A[j] = 0.0f;
+        }
         if (CUTS && cut) A[j] = 0.0f;
     }
     col.set(maps.A(at.b, at.part, s.N), A);
@@ -457,7 +472,7 @@ __global__ void __launch_bounds__(32 * WARPS) join_kernel(const Maps maps, const
     int any = 0;
     auto then = [](float &A, float &H, float a, float h, bool cut) {  // (A, H), then (a, h)
         H = cut ? h : follow(a, h, H);
-        A = cut ? 0.0f : A * a;
+        A = cut ? 0.0f : product(A, a);
     };
     all([&](int i) { then(A, H, pa[i], ph[i], CUTS && (c >> i & 1)); });
     any = c != 0;
