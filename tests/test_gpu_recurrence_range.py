@@ -110,3 +110,28 @@ def test_a_stretch_of_growth_among_ordinary_decays():
         assert torch.isfinite(g).all(), name
         # sums of up to three inputs that overlap within 100 steps of a half each; below 2^-100 nothing counts
         assert float(((g - w).abs() - 1024 * U * w.abs()).max()) <= 2.0**-100, name
+
+
+@pytest.mark.parametrize("form,value", [("decay", 0.5), ("decay", -0.5), ("sigmoid", 0.0)])
+@pytest.mark.parametrize("B,T,N", [(2, 6000, 64), (3, 4000, 9)])
+def test_infinities_stay_where_products_of_decays_underflow(B, T, N, form, value):
+    """An infinite state, input or gradient is infinite, of the definition's sign, to the end (or to the
+    beginning); a decay of 0 makes it NaN. Elsewhere sums of inputs halved from step to step: below 2 in
+    size, 16 u of that."""
+    gen = torch.Generator("cuda").manual_seed(1)
+    a = torch.full((B, T, N), value, device="cuda")
+    x, dh = (torch.rand((B, T, N), device="cuda", generator=gen) for _ in range(2))
+    state, dlast = (torch.rand((B, N), device="cuda", generator=gen) for _ in range(2))
+    inf = float("inf")
+    state[:, 0], state[:, 1] = inf, -inf
+    x[:, 100, 2], x[:, 2500, 3] = inf, -inf
+    dlast[:, 4], dh[:, 2700, 5] = -inf, inf
+    if form == "decay":
+        x[:, 50, 6], a[:, 1999, 6] = inf, 0.0
+        state[:, 7], a[:, 60, 7] = inf, 0.0
+    assert parts(B, T, N, a.dtype, 0) > 1 and parts(B, T, N, a.dtype, 1) > 1
+    h, last, _, dx, dstate = (t.detach().double().cpu() for t in run(a, x, state, dh, dlast, form))
+    rh, rlast, _, rdx, rdstate = definition(a, x, state, dh, dlast, form)
+    assert torch.isinf(rh[..., :4]).any(1).all() and torch.isinf(rdx[..., 4:6]).any(1).all()
+    for name, got, want in (("h", h, rh), ("last", last, rlast), ("dx", dx, rdx), ("dstate", dstate, rdstate)):
+        assert torch.allclose(got, want, rtol=0.0, atol=32 * U, equal_nan=True), name

@@ -130,16 +130,21 @@ __device__ __forceinline__ float keeps() {
     return SIG ? __int_as_float(0x7f800000) : 1.0f;
 }
 
-// s -> A s + H. A state of 0 takes no part where a product of growing decays overflowed; A is not a
-// number where one of them was not finite.
-__device__ __forceinline__ float follow(float A, float H, float s) {
-    return s == 0.0f && !isnan(A) ? H : __fmaf_rn(A, s, H);
-}
-
-// The product of two parts' decays: infinity stands for one that overflowed, which a decay of 0 ends.
+// A product of decays: infinity stands for one that overflowed, kTrace of its sign for one that
+// underflowed (which is still infinite times an infinite state), 0 for one with a decay of 0 in it, and
+// one with a decay that is not finite is not a number.
+constexpr float kTrace = 1.401298464e-45f;
 __device__ __forceinline__ float product(float A, float a) {
     const float p = A * a;
-    return isnan(p) && !isnan(A) && !isnan(a) ? 0.0f : p;
+    if (isnan(p)) return isnan(A) || isnan(a) ? p : 0.0f;
+    return p == 0.0f && A != 0.0f && a != 0.0f ? copysignf(kTrace, p) : p;
+}
+
+// s -> A s + H. A state of 0 takes no part where a product of growing decays overflowed (a finite one
+// takes 1e-45 of itself where a product underflowed).
+__device__ __forceinline__ float follow(float A, float H, float s) {
+    const float r = __fmaf_rn(A, s, H);
+    return isnan(r) && s == 0.0f && !isnan(A) ? H : r;
 }
 
 // The threads of a trial's columns, and the columns of a thread: adjacent ones where rows allow
@@ -424,12 +429,11 @@ __global__ void __launch_bounds__(block_of(WIDE)) maps_kernel(const Args s, cons
     }
 #pragma unroll
     for (int j = 0; j < V; j++) {
-        if (!SIG) {
-            // an infinite decay makes a state of 0 not a number; of finite ones a single 0 makes the product
-            // 0, though it may have overflowed
-            if (isinf(most[j])) A[j] = CUDART_NAN_F;
-            else if (least[j] == 0.0f) A[j] = 0.0f;
-        }
+        // an infinite decay makes a state of 0 not a number; of finite ones a single 0 makes the product 0,
+        // though it may have overflowed; the sigmoid form's are above 0
+        if (!SIG && isinf(most[j])) A[j] = CUDART_NAN_F;
+        else if (!SIG && least[j] == 0.0f) A[j] = 0.0f;
+        else if (A[j] == 0.0f) A[j] = copysignf(kTrace, A[j]);
         if (CUTS && cut) A[j] = 0.0f;
     }
     col.set(maps.A(at.b, at.part, s.N), A);
