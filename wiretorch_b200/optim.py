@@ -290,11 +290,13 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        # asked before any state is made: what a refused capture recorded never runs
+        if torch.cuda.is_current_stream_capturing() and any(
+                p.grad is not None for group in self.param_groups for p in group["params"]):  # fmt: skip
+            raise RuntimeError("AdamW.step cannot be captured into a CUDA graph: its step number is the host's")
         batches, grads = self._current_batches()
         if not batches:
             return loss
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("AdamW.step cannot be captured into a CUDA graph: its step number is the host's")
         device = batches[0].params[0].device
         if device.index == torch.cuda.current_device():
             self._run(batches, grads, device)
