@@ -554,9 +554,8 @@ int wt_grad_norm(const WtGradNorm *a, void *stream);
  * float scale per WT_ADAMW_BLOCK elements, rounded by random bits hashed from (seed, count,
  * the element's number: first[k] + its place). 16-bit tensors have a float master, which is
  * stepped, and the tensor written as its rounding. With `control` (of a wt_grad_norm before
- * it on the stream) the gradients are scaled by its clip and the step is left out when its norm
- * was not finite. The step number of a tensor's bias corrections is step less the steps that were
- * left out: *left[k], where a step that is left out is counted, or control->skipped without `left`. */
+ * it on the stream) the gradients are scaled by its clip, the step is left out when its norm
+ * was not finite, and the step number of the bias corrections is step - control->skipped. */
 typedef struct {
     int32_t n, type, state_bits;
     const uint64_t *p, *g, *m, *v;
@@ -569,7 +568,6 @@ typedef struct {
     int64_t count;                      /* of the random bits */
     uint64_t seed;
     const WtStepControl *control;       /* device, or NULL */
-    const uint64_t *left;               /* an int64 of the device for each tensor, or NULL */
 } WtAdamW;
 
 /* Replaces the optimiser step of the reference's trainer (snn_runners/trainer.py:358-384),

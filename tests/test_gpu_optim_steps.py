@@ -48,79 +48,3 @@ def test_a_refused_capture_leaves_nothing_behind(dtype, bits, max_norm):
         take(ref, other, grads)
     for p, q in zip(ours, other):
         assert torch.equal(p, q) and same_state(opt.state[p], ref.state[q])
-
-
-def left_out(opt, params, grads):
-    """A step that its norm leaves out."""
-    bad = [g.clone() for g in grads]
-    bad[0].view(-1)[0] = float("nan")
-    take(opt, params, bad)
-
-
-@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_steps_that_were_left_out_do_not_count_without_a_limit_either(dtype):
-    """Steps left out, then the limit taken off, or the state loaded by an optimiser without one, a
-    group added: as if the steps that were left out had not been. An optimiser that never had a limit
-    takes its corrections from the host, in 64 bits: 1e-6 of a step of 1e-2 from the device's."""
-    values, more = tensors([1000, (7, 9)], dtype, 1), tensors([33], dtype, 3)
-    grads = [tensors([1000, (7, 9), 33], dtype, 4 + k, 1e-3) for k in range(6)]
-
-    def train(skip, limit, load):
-        ps, qs = params_of(values), params_of(more)
-        opt = optim.AdamW(ps, lr=1e-2, weight_decay=0.0, max_norm=limit)
-        for k in range(2):
-            take(opt, ps, grads[k])
-            for _ in range(3 if skip else 0):
-                left_out(opt, ps, grads[k])
-        assert opt.skipped == (6 if skip else 0)
-        if load:
-            saved, held = opt.state_dict(), opt
-            opt = optim.AdamW(ps, lr=1e-2, weight_decay=0.0)
-            opt.load_state_dict(saved)
-            assert opt.skipped == held.skipped
-        opt.max_norm = None
-        opt.add_param_group({"params": qs, "lr": 1e-2, "weight_decay": 0.0})
-        for k in range(2, 6):
-            take(opt, ps + qs, grads[k])
-        return [opt.state[p].get("master", p).detach() for p in ps + qs]
-
-    want, plain = train(False, 1e6, False), train(False, None, False)
-    for load in (False, True):
-        for p, w, v in zip(train(True, 1e6, load), want, plain):
-            assert torch.equal(p, w)
-            assert bool(((p - v).abs() <= 6 * 2.0**-24 * (40 * 3e-2 + 3 * v.abs())).all())
-
-
-def test_a_step_is_left_out_for_the_tensors_that_had_a_part_in_it():
-    """A tensor that had no gradient in a step that was left out, and one that had."""
-    values = tensors([500, 300], torch.float32, 1)
-    grads = [tensors([500, 300], torch.float32, 4 + k, 1e-3) for k in range(3)]
-    ours, other = params_of(values), params_of(values)
-    opt, ref = (optim.AdamW(ps, lr=1e-2, max_norm=1e6) for ps in (ours, other))
-    for o, ps in ((opt, ours), (ref, other)):
-        take(o, ps, grads[0])
-    ours[1].grad = None
-    ours[0].grad = torch.full_like(ours[0], float("inf"))
-    opt.step()
-    assert opt.state_dict()["wiretorch"]["left"] == [1, 0]
-    for o, ps in ((opt, ours), (ref, other)):
-        take(o, ps[:1], grads[1][:1])
-    assert torch.equal(ours[0], other[0])
-
-
-def test_a_state_without_counts_of_each_tensor_is_loaded():
-    """States that were saved with one count of steps left out for all tensors."""
-    values = tensors([500], torch.float32, 1)
-    grads = [tensors([500], torch.float32, 4 + k, 1e-3) for k in range(3)]
-    ours = params_of(values)
-    opt = optim.AdamW(ours, lr=1e-2, max_norm=1e6)
-    take(opt, ours, grads[0])
-    left_out(opt, ours, grads[0])
-    saved = opt.state_dict()
-    del saved["wiretorch"]["left"]
-    theirs = [torch.nn.Parameter(p.detach().clone()) for p in ours]
-    other = optim.AdamW(theirs, lr=1e-2, max_norm=1e6)
-    other.load_state_dict(saved)
-    for o, ps in ((opt, ours), (other, theirs)):
-        take(o, ps, grads[1])
-    assert torch.equal(ours[0], theirs[0])

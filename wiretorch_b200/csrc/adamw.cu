@@ -22,7 +22,6 @@
 #include <math_constants.h>
 
 #include <cmath>
-#include <cstddef>
 
 #include "common.cuh"
 
@@ -36,9 +35,8 @@ constexpr int kMaxTensors = 320;  // of one launch: the table stays below the 32
 constexpr int kFewTensors = 24;
 
 // What a launch knows of a tensor. first: the number of its first element among all of the
-// optimiser's, each tensor starting on a whole block of kQ. left: the steps it had a part in that were
-// left out, or null. keep: 1 - lr wd. wide: its operands allow access to four elements at once (16
-// bytes, of all of them with 8-bit moments).
+// optimiser's, each tensor starting on a whole block of kQ. keep: 1 - lr wd. wide: its operands
+// allow access to four elements at once (16 bytes, of all of them with 8-bit moments).
 struct __align__(16) Row {
     void *p;
     const void *g;
@@ -46,7 +44,6 @@ struct __align__(16) Row {
     float *m_scale, *v_scale, *master;
     long long numel;
     unsigned long long first;
-    long long *left;
     float lr, keep;
     int wide, type;
 };
@@ -69,11 +66,10 @@ __device__ __forceinline__ const Table<MAX> *as_memory(const Table<MAX> &tb) {
 
 struct Step {
     float b1, c1, b2, c2, eps, minus_zero;
-    float corr1, corr2;    // 1 / (1 - b1^t), 1 / sqrt(1 - b2^t) of tensors without `left`
-    float log_b1, log_b2;  // of others t less what was left out
+    float corr1, corr2;    // 1 / (1 - b1^t), 1 / sqrt(1 - b2^t) when `control` is null
+    float log_b1, log_b2;  // else t = t - control->skipped
     long long t;
     const WtStepControl *control;
-    int counts;  // a step that is left out is counted in the tensors' `left`
     unsigned key0, key1;
 };
 
@@ -178,27 +174,17 @@ struct Rates {
     float clip, corr1, corr2;
 };
 
-// False when the step is to be left out (the norm was not finite); block 0 counts it then.
-template <int MAX>
-__device__ __forceinline__ bool clip_of(const Table<MAX> &table, const Step &s, float &clip) {
-    clip = 1.0f;
-    if (!s.control) return true;
-    if (!s.control->skip) {
-        clip = s.control->clip;
-        return true;
+// False when the step is to be left out (the norm was not finite).
+__device__ __forceinline__ bool rates_of(const Step &s, Rates &r) {
+    r = Rates{1.0f, s.corr1, s.corr2};
+    if (s.control) {
+        if (s.control->skip) return false;
+        const float t = (float)(s.t - s.control->skipped);
+        r.clip = s.control->clip;
+        r.corr1 = 1.0f / -expm1f(t * s.log_b1);
+        r.corr2 = rsqrtf(-expm1f(t * s.log_b2));
     }
-    if (s.counts && blockIdx.x == 0) {
-        const Table<MAX> *tb = as_memory(table);
-        for (int k = threadIdx.x; k < table.n; k += kThreads)
-            if (tb->row[k].numel) *tb->row[k].left += 1;
-    }
-    return false;
-}
-
-__device__ __forceinline__ Rates rates_of(const Row &row, const Step &s, float clip) {
-    if (!row.left) return Rates{clip, s.corr1, s.corr2};
-    const float t = (float)(s.t - *row.left);
-    return Rates{clip, 1.0f / -expm1f(t * s.log_b1), rsqrtf(-expm1f(t * s.log_b2))};
+    return true;
 }
 
 // The root and the reciprocal are the hardware's (one and two units in the last place): an error
@@ -245,10 +231,9 @@ __device__ __forceinline__ void advance(float g, float &m, float &v, const Step 
 // 150 bf16 tensors of 30M elements 131 us, 6.4 TB/s.
 template <typename P, int MAX>
 __global__ void __launch_bounds__(kThreads, 5) adamw32(const __grid_constant__ Table<MAX> tb, const __grid_constant__ Step s) {
-    float clip;
-    if (!clip_of(tb, s, clip)) return;
+    Rates r;
+    if (!rates_of(s, r)) return;
     run_of_chunks(tb, block_of(s), [&](const Row &t, long long first, long long end) {
-        const Rates r = rates_of(t, s, clip);
         constexpr bool kMaster = sizeof(P) == 2;
         P *const p = static_cast<P *>(t.p);
         const P *const g = static_cast<const P *>(t.g);
@@ -468,10 +453,9 @@ struct __align__(16) Slot {
 template <typename P, int MAX>
 __global__ void __launch_bounds__(kThreads, 4) adamw8(const __grid_constant__ Table<MAX> tb, const __grid_constant__ Step s) {
     __shared__ Slot<P> slots[kThreads / 32][2];
-    float clip;
-    if (!clip_of(tb, s, clip)) return;
+    Rates r;
+    if (!rates_of(s, r)) return;
     run_of_chunks(tb, block_of(s), [&](const Row &t, long long first, long long end) {
-        const Rates r = rates_of(t, s, clip);
         P *const p = static_cast<P *>(t.p);
         float *const master = sizeof(P) == 2 ? t.master : reinterpret_cast<float *>(p);
         const P *const g = static_cast<const P *>(t.g);
@@ -625,7 +609,6 @@ void fill(Table<MAX> &tb, const WtAdamW &a, int from, int n) {
     unsigned chunks = 0;
     tb.n = n;
     const int z = a.type == WT_F32 || a.state_bits == 8 ? 16 : 8;
-    long long *const skipped = a.control ? (long long *)((char *)a.control + offsetof(WtStepControl, skipped)) : nullptr;
     for (int i = 0; i < n; i++) {
         const int k = from + i;
         Row &t = tb.row[i];
@@ -638,7 +621,6 @@ void fill(Table<MAX> &tb, const WtAdamW &a, int from, int n) {
         t.master = a.master ? (float *)a.master[k] : nullptr;
         t.numel = a.numel[k];
         t.first = a.first ? (unsigned long long)a.first[k] : 0;
-        t.left = a.left ? (long long *)a.left[k] : skipped;
         t.lr = (float)a.lr[k];
         t.keep = (float)(1.0 - a.lr[k] * a.weight_decay[k]);
         t.type = a.type;
@@ -674,7 +656,6 @@ Step step_of(const WtAdamW &a) {
     s.log_b2 = (float)std::log(a.beta2);
     s.t = a.step;
     s.control = a.control;
-    s.counts = a.left != nullptr;
     s.key0 = mix_host((unsigned)(2 * a.count), (unsigned)a.seed, 0x3C6EF372u);
     s.key1 = mix_host((unsigned)(2 * a.count + 1), (unsigned)a.seed, 0x3C6EF372u);
     return s;

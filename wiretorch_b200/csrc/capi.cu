@@ -356,7 +356,7 @@ int wt_adamw_step(const WtAdamW *a, void *stream) {
         if (a->state_bits == 8 && (a->first[k] < 0 || a->first[k] % WT_ADAMW_BLOCK))
             return fail(WT_ERR_ARGS, "a tensor's first number must be that of a whole block%s");
         if (!a->numel[k]) continue;
-        if (!a->p[k] || !a->g[k] || !a->m[k] || !a->v[k] || (a->type != WT_F32 && !a->master[k]) || (a->left && !a->left[k]) ||
+        if (!a->p[k] || !a->g[k] || !a->m[k] || !a->v[k] || (a->type != WT_F32 && !a->master[k]) ||
             (a->state_bits == 8 && (!a->m_scale[k] || !a->v_scale[k])))
             return fail(WT_ERR_ARGS, "missing AdamW buffers%s");
     }

@@ -39,7 +39,6 @@ class _AdamW(_C.Structure):
         ("numel", _lib.P), ("first", _lib.P), ("lr", _lib.P), ("weight_decay", _lib.P),
         ("beta1", _C.c_double), ("beta2", _C.c_double), ("eps", _C.c_double),
         ("step", _C.c_int64), ("count", _C.c_int64), ("seed", _C.c_uint64), ("control", _lib.P),
-        ("left", _lib.P),
     ]  # fmt: skip
 
 
@@ -81,17 +80,15 @@ class _Batch:
 
     def __init__(self, dtype, betas, eps, born):
         self.dtype, self.betas, self.eps, self.born = dtype, betas, eps, born
-        self.params, self.held, self.groups, self.first, self.numel, self.slots = [], [], [], [], [], []
-        self.left = None
+        self.params, self.held, self.groups, self.first, self.numel = [], [], [], [], []
         self.strided = False  # a tensor in another order than its dimensions'
 
-    def add(self, p, held, group, first, slot):
+    def add(self, p, held, group, first):
         self.params.append(p)
         self.held.append(held)
         self.groups.append(group)
         self.first.append(first)
         self.numel.append(p.numel())
-        self.slots.append(slot)
         self.strided |= not p.is_contiguous()
 
     def close(self, names):
@@ -114,12 +111,6 @@ class _Batch:
     def takes(self, grads):
         """Whether the gradients can be read as they are."""
         return not self.strided and self._as_planned(grads)
-
-    def left_in(self, counts):
-        """The addresses of the tensors' counts."""
-        if self.left is None or self.left[0] is not counts:
-            self.left = counts, array("Q", [counts.data_ptr() + 8 * slot for slot in self.slots])
-        return self.left[1]
 
     def rates(self, name):
         groups = self.groups
@@ -149,8 +140,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"max_norm must be above 0, not {max_norm}")
         self.state_bits, self.max_norm, self.seed = state_bits, max_norm, int(seed) & 0xFFFFFFFF
         self.steps = 0
-        self._control = self._partial = self._batches = self._left = None
-        self._slots = {}  # of each tensor, its place in _left
+        self._control = self._partial = self._batches = None
         super().__init__(params, {"lr": lr, "betas": betas, "eps": eps, "weight_decay": weight_decay})
 
     def add_param_group(self, param_group):
@@ -161,7 +151,7 @@ class AdamW(torch.optim.Optimizer):
         except Exception:
             self.param_groups.pop()
             raise
-        group.setdefault("born", self.steps)
+        group.setdefault("born", self.steps - self.skipped)
 
     def _check_group(self, group):
         (b1, b2), eps = group["betas"], group["eps"]
@@ -190,14 +180,6 @@ class AdamW(torch.optim.Optimizer):
         if self._control is None:
             self._control = torch.zeros(6, dtype=torch.int32, device=device)
         return self._control
-
-    def _left_of(self, device):
-        """A count of each tensor, on the device: the steps it had a part in that were left out."""
-        if self._left is None or self._left.numel() < len(self._slots):
-            old, self._left = self._left, torch.zeros(len(self._slots), dtype=torch.int64, device=device)
-            if old is not None:
-                self._left[: old.numel()] = old
-        return self._left
 
     @property
     def grad_norm(self):
@@ -258,7 +240,7 @@ class AdamW(torch.optim.Optimizer):
                     kind = (p.dtype, *key)
                     if kind not in batches:
                         batches[kind] = _Batch(*kind)
-                    batches[kind].add(p, self._checked_state(p), group, at, self._slots.setdefault(p, len(self._slots)))
+                    batches[kind].add(p, self._checked_state(p), group, at)
         for batch in batches.values():
             names = ["exp_avg", "exp_avg_sq"] + (["exp_avg_scale", "exp_avg_sq_scale"] if eight else [])
             batch.close(names + (["master"] if batch.dtype != torch.float32 else []))
@@ -328,8 +310,6 @@ class AdamW(torch.optim.Optimizer):
         at = [_addresses(gs) for gs in grads]
         if self.max_norm is not None:
             self._norm(batches, at, device, stream)
-        if self.max_norm is not None or self._left is not None:  # what was left out counts on without a limit, too
-            self._left_of(device)
         self.steps += 1
         for batch, g in zip(batches, at):
             self._launch(batch, g, stream)
@@ -367,8 +347,6 @@ class AdamW(torch.optim.Optimizer):
         a.step, a.count, a.seed = self.steps - batch.born, self.steps, self.seed
         if self.max_norm is not None:
             a.control = self._control.data_ptr()
-        if self._left is not None:
-            a.left = _at(batch.left_in(self._left))
         with _lib.timed("wt_adamw_step"):
             rc = _lib.lib().wt_adamw_step(_C.byref(a), stream)
         _lib.check(rc, "wt_adamw_step")
@@ -377,11 +355,8 @@ class AdamW(torch.optim.Optimizer):
     # --- saving ---
 
     def state_dict(self):
-        left = [0] * len(self._slots) if self._left is None else self._left.tolist()
-        of = [self._slots.get(p, len(left)) for group in self.param_groups for p in group["params"]]
-        return super().state_dict() | {"wiretorch": {
-            "state_bits": self.state_bits, "seed": self.seed, "steps": self.steps, "skipped": self.skipped,
-            "left": [left[slot] if slot < len(left) else 0 for slot in of]}}  # fmt: skip
+        return super().state_dict() | {"wiretorch": {"state_bits": self.state_bits, "seed": self.seed,
+                                                     "steps": self.steps, "skipped": self.skipped}}  # fmt: skip
 
     def load_state_dict(self, state_dict):
         own = state_dict.get("wiretorch")
@@ -400,13 +375,9 @@ class AdamW(torch.optim.Optimizer):
         self.steps, self.seed = own["steps"], own["seed"]
         if own["skipped"] or self._control is not None:
             self._control_of(self._device())[4:].view(torch.int64).fill_(own["skipped"])
-        left = own.get("left", [own["skipped"]] * len(params))  # without the list: of all tensors alike
-        self._slots, self._left = {p: slot for slot, p in enumerate(params)}, None
-        if any(left):
-            self._left = torch.tensor(left, dtype=torch.int64, device=self._device())
 
     def __getstate__(self):
-        own = ("state_bits", "max_norm", "seed", "steps", "_control", "_left", "_slots")
+        own = ("state_bits", "max_norm", "seed", "steps", "_control")
         return super().__getstate__() | {k: getattr(self, k) for k in own}
 
     def __setstate__(self, state):
