@@ -554,8 +554,9 @@ int wt_grad_norm(const WtGradNorm *a, void *stream);
  * float scale per WT_ADAMW_BLOCK elements, rounded by random bits hashed from (seed, count,
  * the element's number: first[k] + its place). 16-bit tensors have a float master, which is
  * stepped, and the tensor written as its rounding. With `control` (of a wt_grad_norm before
- * it on the stream) the gradients are scaled by its clip, the step is left out when its norm
- * was not finite, and the step number of the bias corrections is step - control->skipped. */
+ * it on the stream) the gradients are scaled by its clip and the step is left out when its norm
+ * was not finite. The step number of the bias corrections is step - *skipped, the steps left out so
+ * far; control->skipped without `skipped`, step without either. */
 typedef struct {
     int32_t n, type, state_bits;
     const uint64_t *p, *g, *m, *v;
@@ -568,6 +569,7 @@ typedef struct {
     int64_t count;                      /* of the random bits */
     uint64_t seed;
     const WtStepControl *control;       /* device, or NULL */
+    const int64_t *skipped;             /* device, or NULL */
 } WtAdamW;
 
 /* Replaces the optimiser step of the reference's trainer (snn_runners/trainer.py:358-384),

@@ -48,3 +48,45 @@ def test_a_refused_capture_leaves_nothing_behind(dtype, bits, max_norm):
         take(ref, other, grads)
     for p, q in zip(ours, other):
         assert torch.equal(p, q) and same_state(opt.state[p], ref.state[q])
+
+
+def left_out(opt, params, grads):
+    """A step that its norm leaves out."""
+    bad = [g.clone() for g in grads]
+    bad[0].view(-1)[0] = float("nan")
+    take(opt, params, bad)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_steps_that_were_left_out_do_not_count_without_a_limit_either(dtype):
+    """Steps left out, then the limit taken off, or the state loaded by an optimiser without one, a
+    group added: as if the steps that were left out had not been. An optimiser that never had a limit takes
+    its corrections from the host, in 64 bits: the steps, of at most 3e-2, agree within 40 u of themselves and
+    the parameter's own roundings, 3 u of it in each (u = 2^-24)."""
+    values, more = tensors([1000, (7, 9)], dtype, 1), tensors([33], dtype, 3)
+    grads = [tensors([1000, (7, 9), 33], dtype, 4 + k, 1e-3) for k in range(6)]
+
+    def train(skip, limit, load):
+        ps, qs = params_of(values), params_of(more)
+        opt = optim.AdamW(ps, lr=1e-2, weight_decay=0.0, max_norm=limit)
+        for k in range(2):
+            take(opt, ps, grads[k])
+            for _ in range(3 if skip else 0):
+                left_out(opt, ps, grads[k])
+        assert opt.skipped == (6 if skip else 0)
+        if load:
+            saved, held = opt.state_dict(), opt
+            opt = optim.AdamW(ps, lr=1e-2, weight_decay=0.0)
+            opt.load_state_dict(saved)
+            assert opt.skipped == held.skipped
+        opt.max_norm = None
+        opt.add_param_group({"params": qs, "lr": 1e-2, "weight_decay": 0.0})
+        for k in range(2, 6):
+            take(opt, ps + qs, grads[k])
+        return [opt.state[p].get("master", p).detach() for p in ps + qs]
+
+    want, plain = train(False, 1e6, False), train(False, None, False)
+    for load in (False, True):
+        for p, w, v in zip(train(True, 1e6, load), want, plain):
+            assert torch.equal(p, w)
+            assert bool(((p - v).abs() <= 6 * 2.0**-24 * (40 * 3e-2 + 3 * v.abs())).all())

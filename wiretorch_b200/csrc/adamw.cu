@@ -22,6 +22,7 @@
 #include <math_constants.h>
 
 #include <cmath>
+#include <cstddef>
 
 #include "common.cuh"
 
@@ -66,10 +67,11 @@ __device__ __forceinline__ const Table<MAX> *as_memory(const Table<MAX> &tb) {
 
 struct Step {
     float b1, c1, b2, c2, eps, minus_zero;
-    float corr1, corr2;    // 1 / (1 - b1^t), 1 / sqrt(1 - b2^t) when `control` is null
-    float log_b1, log_b2;  // else t = t - control->skipped
+    float corr1, corr2;    // 1 / (1 - b1^t), 1 / sqrt(1 - b2^t) when `skipped` is null
+    float log_b1, log_b2;  // else t = t - *skipped
     long long t;
     const WtStepControl *control;
+    const long long *skipped;
     unsigned key0, key1;
 };
 
@@ -179,8 +181,10 @@ __device__ __forceinline__ bool rates_of(const Step &s, Rates &r) {
     r = Rates{1.0f, s.corr1, s.corr2};
     if (s.control) {
         if (s.control->skip) return false;
-        const float t = (float)(s.t - s.control->skipped);
         r.clip = s.control->clip;
+    }
+    if (s.skipped) {
+        const float t = (float)(s.t - *s.skipped);
         r.corr1 = 1.0f / -expm1f(t * s.log_b1);
         r.corr2 = rsqrtf(-expm1f(t * s.log_b2));
     }
@@ -656,6 +660,8 @@ Step step_of(const WtAdamW &a) {
     s.log_b2 = (float)std::log(a.beta2);
     s.t = a.step;
     s.control = a.control;
+    if (a.skipped) s.skipped = (const long long *)a.skipped;
+    else if (a.control) s.skipped = (const long long *)((const char *)a.control + offsetof(WtStepControl, skipped));
     s.key0 = mix_host((unsigned)(2 * a.count), (unsigned)a.seed, 0x3C6EF372u);
     s.key1 = mix_host((unsigned)(2 * a.count + 1), (unsigned)a.seed, 0x3C6EF372u);
     return s;

@@ -20,6 +20,7 @@ import torch
 from wiretorch_b200 import _lib
 
 BLOCK = 256  # WT_ADAMW_BLOCK: elements that share a scale of the 8-bit moments
+SKIPPED = 16  # offsetof(WtStepControl, skipped)
 _C = _lib.C
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # WT_F32, WT_BF16, WT_F16
 
@@ -39,6 +40,7 @@ class _AdamW(_C.Structure):
         ("numel", _lib.P), ("first", _lib.P), ("lr", _lib.P), ("weight_decay", _lib.P),
         ("beta1", _C.c_double), ("beta2", _C.c_double), ("eps", _C.c_double),
         ("step", _C.c_int64), ("count", _C.c_int64), ("seed", _C.c_uint64), ("control", _lib.P),
+        ("skipped", _lib.P),
     ]  # fmt: skip
 
 
@@ -189,7 +191,7 @@ class AdamW(torch.optim.Optimizer):
     @property
     def skipped(self) -> int:
         """Steps left out so far (reads the device)."""
-        return 0 if self._control is None else int(self._control[4:].view(torch.int64))
+        return 0 if self._control is None else int(self._control[SKIPPED // 4 :].view(torch.int64))
 
     # --- state ---
 
@@ -345,8 +347,9 @@ class AdamW(torch.optim.Optimizer):
         a.numel, a.first, a.lr, a.weight_decay = _at(batch.counts), _at(batch.firsts), _at(lr), _at(decay)
         (a.beta1, a.beta2), a.eps = batch.betas, batch.eps
         a.step, a.count, a.seed = self.steps - batch.born, self.steps, self.seed
-        if self.max_norm is not None:
-            a.control = self._control.data_ptr()
+        if self._control is not None:  # what was left out counts on without a limit, too
+            at = self._control.data_ptr()
+            a.control, a.skipped = None if self.max_norm is None else at, at + SKIPPED
         with _lib.timed("wt_adamw_step"):
             rc = _lib.lib().wt_adamw_step(_C.byref(a), stream)
         _lib.check(rc, "wt_adamw_step")
@@ -374,7 +377,7 @@ class AdamW(torch.optim.Optimizer):
         self._batches = None
         self.steps, self.seed = own["steps"], own["seed"]
         if own["skipped"] or self._control is not None:
-            self._control_of(self._device())[4:].view(torch.int64).fill_(own["skipped"])
+            self._control_of(self._device())[SKIPPED // 4 :].view(torch.int64).fill_(own["skipped"])
 
     def __getstate__(self):
         own = ("state_bits", "max_norm", "seed", "steps", "_control")
