@@ -556,7 +556,8 @@ int wt_grad_norm(const WtGradNorm *a, void *stream);
  * stepped, and the tensor written as its rounding. With `control` (of a wt_grad_norm before
  * it on the stream) the gradients are scaled by its clip and the step is left out when its norm
  * was not finite. The step number of the bias corrections is step - *skipped, the steps left out so
- * far; control->skipped without `skipped`, step without either. */
+ * far (control->skipped without `skipped`, 0 without either), less what a tensor has in `before`: the
+ * steps, but for those left out, before its first. */
 typedef struct {
     int32_t n, type, state_bits;
     const uint64_t *p, *g, *m, *v;
@@ -570,6 +571,7 @@ typedef struct {
     uint64_t seed;
     const WtStepControl *control;       /* device, or NULL */
     const int64_t *skipped;             /* device, or NULL */
+    const uint64_t *before;             /* an int64 of the device for each tensor or 0, or NULL */
 } WtAdamW;
 
 /* Replaces the optimiser step of the reference's trainer (snn_runners/trainer.py:358-384),

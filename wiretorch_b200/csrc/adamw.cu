@@ -36,8 +36,9 @@ constexpr int kMaxTensors = 320;  // of one launch: the table stays below the 32
 constexpr int kFewTensors = 24;
 
 // What a launch knows of a tensor. first: the number of its first element among all of the
-// optimiser's, each tensor starting on a whole block of kQ. keep: 1 - lr wd. wide: its operands
-// allow access to four elements at once (16 bytes, of all of them with 8-bit moments).
+// optimiser's, each tensor starting on a whole block of kQ. before: the steps before the tensor's
+// first, or null. keep: 1 - lr wd. wide: its operands allow access to four elements at once (16
+// bytes, of all of them with 8-bit moments).
 struct __align__(16) Row {
     void *p;
     const void *g;
@@ -45,6 +46,7 @@ struct __align__(16) Row {
     float *m_scale, *v_scale, *master;
     long long numel;
     unsigned long long first;
+    const long long *before;
     float lr, keep;
     int wide, type;
 };
@@ -67,8 +69,8 @@ __device__ __forceinline__ const Table<MAX> *as_memory(const Table<MAX> &tb) {
 
 struct Step {
     float b1, c1, b2, c2, eps, minus_zero;
-    float corr1, corr2;    // 1 / (1 - b1^t), 1 / sqrt(1 - b2^t) when `skipped` is null
-    float log_b1, log_b2;  // else t = t - *skipped
+    float corr1, corr2;    // 1 / (1 - b1^t), 1 / sqrt(1 - b2^t) of tensors without `before` when `skipped` is null
+    float log_b1, log_b2;  // else t - *skipped - *before takes the place of t
     long long t;
     const WtStepControl *control;
     const long long *skipped;
@@ -177,18 +179,15 @@ struct Rates {
 };
 
 // False when the step is to be left out (the norm was not finite).
-__device__ __forceinline__ bool rates_of(const Step &s, Rates &r) {
-    r = Rates{1.0f, s.corr1, s.corr2};
-    if (s.control) {
-        if (s.control->skip) return false;
-        r.clip = s.control->clip;
-    }
-    if (s.skipped) {
-        const float t = (float)(s.t - *s.skipped);
-        r.corr1 = 1.0f / -expm1f(t * s.log_b1);
-        r.corr2 = rsqrtf(-expm1f(t * s.log_b2));
-    }
-    return true;
+__device__ __forceinline__ bool clip_of(const Step &s, float &clip) {
+    clip = s.control ? s.control->clip : 1.0f;
+    return !s.control || !s.control->skip;
+}
+
+__device__ __forceinline__ Rates rates_of(const Row &row, const Step &s, float clip) {
+    if (!s.skipped && !row.before) return Rates{clip, s.corr1, s.corr2};
+    const float t = (float)(s.t - (s.skipped ? *s.skipped : 0) - (row.before ? *row.before : 0));
+    return Rates{clip, 1.0f / -expm1f(t * s.log_b1), rsqrtf(-expm1f(t * s.log_b2))};
 }
 
 // The root and the reciprocal are the hardware's (one and two units in the last place): an error
@@ -235,9 +234,10 @@ __device__ __forceinline__ void advance(float g, float &m, float &v, const Step 
 // 150 bf16 tensors of 30M elements 131 us, 6.4 TB/s.
 template <typename P, int MAX>
 __global__ void __launch_bounds__(kThreads, 5) adamw32(const __grid_constant__ Table<MAX> tb, const __grid_constant__ Step s) {
-    Rates r;
-    if (!rates_of(s, r)) return;
+    float clip;
+    if (!clip_of(s, clip)) return;
     run_of_chunks(tb, block_of(s), [&](const Row &t, long long first, long long end) {
+        const Rates r = rates_of(t, s, clip);
         constexpr bool kMaster = sizeof(P) == 2;
         P *const p = static_cast<P *>(t.p);
         const P *const g = static_cast<const P *>(t.g);
@@ -457,9 +457,10 @@ struct __align__(16) Slot {
 template <typename P, int MAX>
 __global__ void __launch_bounds__(kThreads, 4) adamw8(const __grid_constant__ Table<MAX> tb, const __grid_constant__ Step s) {
     __shared__ Slot<P> slots[kThreads / 32][2];
-    Rates r;
-    if (!rates_of(s, r)) return;
+    float clip;
+    if (!clip_of(s, clip)) return;
     run_of_chunks(tb, block_of(s), [&](const Row &t, long long first, long long end) {
+        const Rates r = rates_of(t, s, clip);
         P *const p = static_cast<P *>(t.p);
         float *const master = sizeof(P) == 2 ? t.master : reinterpret_cast<float *>(p);
         const P *const g = static_cast<const P *>(t.g);
@@ -625,6 +626,7 @@ void fill(Table<MAX> &tb, const WtAdamW &a, int from, int n) {
         t.master = a.master ? (float *)a.master[k] : nullptr;
         t.numel = a.numel[k];
         t.first = a.first ? (unsigned long long)a.first[k] : 0;
+        t.before = a.before ? (const long long *)a.before[k] : nullptr;
         t.lr = (float)a.lr[k];
         t.keep = (float)(1.0 - a.lr[k] * a.weight_decay[k]);
         t.type = a.type;

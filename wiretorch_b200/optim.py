@@ -40,7 +40,7 @@ class _AdamW(_C.Structure):
         ("numel", _lib.P), ("first", _lib.P), ("lr", _lib.P), ("weight_decay", _lib.P),
         ("beta1", _C.c_double), ("beta2", _C.c_double), ("eps", _C.c_double),
         ("step", _C.c_int64), ("count", _C.c_int64), ("seed", _C.c_uint64), ("control", _lib.P),
-        ("skipped", _lib.P),
+        ("skipped", _lib.P), ("before", _lib.P),
     ]  # fmt: skip
 
 
@@ -77,11 +77,11 @@ def _same(a, b):
 
 
 class _Batch:
-    """The tensors that one call steps, those of one type, betas, eps and age, with the objects
-    that were checked when it was made; their addresses are read anew in every step."""
+    """The tensors that one call steps, those of one type, betas and eps, with the objects that
+    were checked when it was made; their addresses are read anew in every step."""
 
-    def __init__(self, dtype, betas, eps, born):
-        self.dtype, self.betas, self.eps, self.born = dtype, betas, eps, born
+    def __init__(self, dtype, betas, eps):
+        self.dtype, self.betas, self.eps = dtype, betas, eps
         self.params, self.held, self.groups, self.first, self.numel = [], [], [], [], []
         self.strided = False  # a tensor in another order than its dimensions'
 
@@ -95,6 +95,7 @@ class _Batch:
 
     def close(self, names):
         self.state = {name: [h[name] for h in self.held] for name in names}
+        self.before = [h.get("before") for h in self.held] if any("before" in h for h in self.held) else None
         self.types = array("i", [TYPES[self.dtype]]) * len(self.params)
         self.counts, self.firsts = array("q", self.numel), array("q", self.first)
         self.index = self.params[0].get_device()
@@ -130,9 +131,10 @@ class AdamW(torch.optim.Optimizer):
     all gradients (``grad_norm``, a device tensor, holds the last one); with it a step whose
     norm is not finite changes nothing and does not count. ``seed``: of the 8-bit rounding.
 
-    The step number is the optimiser's (a group added later counts from there); a tensor
-    without a gradient is left as it is. The step runs on the current stream and does not
-    synchronise; it cannot be captured into a CUDA graph (the step number is the host's)."""
+    The step number is the optimiser's, counted from a tensor's first step, the one of its first gradient
+    (``before`` in its state holds the steps before); a tensor without a gradient is left as it is. The
+    step runs on the current stream and does not synchronise; it cannot be captured into a CUDA
+    graph (the step number is the host's)."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32,
                  max_norm=None, seed=0):  # fmt: skip
@@ -153,7 +155,6 @@ class AdamW(torch.optim.Optimizer):
         except Exception:
             self.param_groups.pop()
             raise
-        group.setdefault("born", self.steps - self.skipped)
 
     def _check_group(self, group):
         (b1, b2), eps = group["betas"], group["eps"]
@@ -188,10 +189,13 @@ class AdamW(torch.optim.Optimizer):
         """The last step's gradient norm before clipping, a device tensor (None without max_norm)."""
         return None if self._control is None else self._control[:1].view(torch.float32)[0]
 
+    def _skipped_at(self):
+        return self._control[SKIPPED // 4 :].view(torch.int64)
+
     @property
     def skipped(self) -> int:
         """Steps left out so far (reads the device)."""
-        return 0 if self._control is None else int(self._control[SKIPPED // 4 :].view(torch.int64))
+        return 0 if self._control is None else int(self._skipped_at())
 
     # --- state ---
 
@@ -208,6 +212,10 @@ class AdamW(torch.optim.Optimizer):
                     held[name + "_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
             if p.dtype != torch.float32:
                 held["master"] = p.detach().float()
+            if self.steps:
+                held["before"] = torch.full((1,), self.steps, dtype=torch.int64, device=p.device)
+                if self._control is not None:
+                    held["before"] -= self._skipped_at()
         return held
 
     def _checked_state(self, p):
@@ -218,6 +226,9 @@ class AdamW(torch.optim.Optimizer):
         names = [("exp_avg", kind), ("exp_avg_sq", kind)]
         if p.dtype != torch.float32:
             names.append(("master", torch.float32))
+        before = held.get("before")
+        if before is not None and (before.dtype != torch.int64 or before.numel() != 1 or before.device != p.device):
+            raise ValueError("the state's before must be one int64 on its tensor's device")
         for name, want in names:
             t = held[name]
             if t.dtype != want or t.shape != p.shape or t.device != p.device or t.stride() != p.stride():
@@ -234,7 +245,7 @@ class AdamW(torch.optim.Optimizer):
         eight, batches, first = self.state_bits == 8, {}, 0
         for group in self.param_groups:
             self._check_group(group)
-            key = (tuple(group["betas"]), group["eps"], group["born"])
+            key = (tuple(group["betas"]), group["eps"])
             for p in group["params"]:
                 at = first
                 first += -(-p.numel() // BLOCK) * BLOCK
@@ -260,7 +271,7 @@ class AdamW(torch.optim.Optimizer):
         if not all(map(is_not, grads, repeat(None))):
             params = [p for p, g in zip(params, grads) if g is not None]
             grads = [g for g in grads if g is not None]
-        settings = [(group["betas"], group["eps"], group["born"], len(group["params"])) for group in self.param_groups]
+        settings = [(group["betas"], group["eps"], len(group["params"])) for group in self.param_groups]
         if (held is None or held[0] != settings or not _same(held[1], params) or not _same(held[3], self._state_now())
                 or not all(map(_Batch.is_current, held[2]))):  # fmt: skip
             batches = self._plan(set(params))
@@ -346,7 +357,10 @@ class AdamW(torch.optim.Optimizer):
             a.master = _at(state["master"])
         a.numel, a.first, a.lr, a.weight_decay = _at(batch.counts), _at(batch.firsts), _at(lr), _at(decay)
         (a.beta1, a.beta2), a.eps = batch.betas, batch.eps
-        a.step, a.count, a.seed = self.steps - batch.born, self.steps, self.seed
+        a.step, a.count, a.seed = self.steps, self.steps, self.seed
+        if batch.before is not None:
+            before = array("Q", [0 if t is None else t.data_ptr() for t in batch.before])
+            a.before = _at(before)
         if self._control is not None:  # what was left out counts on without a limit, too
             at = self._control.data_ptr()
             a.control, a.skipped = None if self.max_norm is None else at, at + SKIPPED
@@ -374,10 +388,16 @@ class AdamW(torch.optim.Optimizer):
         for i, p in zip(ids, params):
             if i in state_dict["state"]:
                 self.state[p] = {k: t.detach().to(p.device, copy=True) for k, t in state_dict["state"][i].items()}
+        for group in self.param_groups:  # a state that has the steps before a group was added with the group
+            born = group.pop("born", 0)
+            for p in group["params"] if born else ():
+                if self.state.get(p):
+                    self.state[p].setdefault("before", torch.full((1,), born, dtype=torch.int64, device=p.device))
         self._batches = None
         self.steps, self.seed = own["steps"], own["seed"]
         if own["skipped"] or self._control is not None:
-            self._control_of(self._device())[SKIPPED // 4 :].view(torch.int64).fill_(own["skipped"])
+            self._control_of(self._device())
+            self._skipped_at().fill_(own["skipped"])
 
     def __getstate__(self):
         own = ("state_bits", "max_norm", "seed", "steps", "_control")
