@@ -180,3 +180,45 @@ def test_groups_that_were_used_before_and_states_that_count_by_group():
         assert torch.equal(p, q)
     for p, q in zip(new, ref.param_groups[0]["params"]):
         assert torch.equal(p, q)
+
+
+def test_settings_that_change_between_steps_are_taken():
+    """A group's dict put in the place of another with other rates, betas changed within their list."""
+    values = tensors([300], torch.float32, 1)
+    grads = [tensors([300], torch.float32, 4 + k, 1e-3) for k in range(4)]
+    (p,), (q,) = params_of(values), params_of(values)
+    opt = optim.AdamW([p], lr=1e-2, betas=[0.9, 0.999])
+    ref = optim.AdamW([q], lr=1e-2, betas=(0.9, 0.999))
+    for k in range(4):
+        if k == 1:
+            opt.param_groups[0] = {**opt.param_groups[0], "lr": 1e-3, "weight_decay": 0.5}
+            ref.param_groups[0].update(lr=1e-3, weight_decay=0.5)
+        if k == 2:
+            opt.param_groups = [dict(group, lr=0.0) for group in opt.param_groups]
+            ref.param_groups[0]["lr"] = 0.0
+        if k == 3:
+            opt.param_groups[0]["lr"] = ref.param_groups[0]["lr"] = 1e-2
+            opt.param_groups[0]["betas"][0] = 0.5
+            ref.param_groups[0]["betas"] = (0.5, 0.999)
+        take(opt, [p], grads[k])
+        take(ref, [q], grads[k])
+        assert torch.equal(p, q), k
+
+
+def test_tensors_without_a_gradient_keep_their_numbers():
+    """What the 8-bit rounding numbers an element by includes the tensors ahead that have no gradient: one
+    of another size in their place, and the numbers follow."""
+    (v, g) = tensors([500, 500], torch.float32, 1)
+    ahead = tensors([300, 900], torch.float32, 2)
+    p = torch.nn.Parameter(v.clone())
+    first, second = params_of(ahead)
+    opt = optim.AdamW([first, p], state_bits=8)
+    take(opt, [p], [g])
+    q = torch.nn.Parameter(p.detach().clone())
+    ref = optim.AdamW([second, q], state_bits=8)
+    ref.state[q] = {k: t.clone() for k, t in opt.state[p].items()}
+    ref.steps = 1
+    opt.param_groups[0]["params"][0] = second
+    take(opt, [p], [g])
+    take(ref, [q], [g])
+    assert torch.equal(p, q) and same_state(opt.state[p], ref.state[q])

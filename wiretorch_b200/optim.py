@@ -265,18 +265,19 @@ class AdamW(torch.optim.Optimizer):
     def _current_batches(self):
         """The batches of the tensors that have a gradient now: the last step's, where nothing but
         gradients and rates changed since, and their gradients, in the order of each tensor's memory."""
-        held = self._batches
-        params = [p for group in self.param_groups for p in group["params"]]
+        held, groups = self._batches, self.param_groups
+        every = params = [p for group in groups for p in group["params"]]
         grads = list(map(_grad, params))
         if not all(map(is_not, grads, repeat(None))):
             params = [p for p, g in zip(params, grads) if g is not None]
             grads = [g for g in grads if g is not None]
-        settings = [(group["betas"], group["eps"], len(group["params"])) for group in self.param_groups]
-        if (held is None or held[0] != settings or not _same(held[1], params) or not _same(held[3], self._state_now())
-                or not all(map(_Batch.is_current, held[2]))):  # fmt: skip
+        settings = [(tuple(group["betas"]), group["eps"], len(group["params"])) for group in groups]
+        if (held is None or held[0] != settings or not _same(held[1], groups) or not _same(held[2], every)
+                or not (params is every and held[3] is held[2] or _same(held[3], params))
+                or not _same(held[5], self._state_now()) or not all(map(_Batch.is_current, held[4]))):  # fmt: skip
             batches = self._plan(set(params))
-            held = self._batches = (settings, params, batches, self._state_now())
-        batches = held[2]
+            held = self._batches = (settings, list(groups), every, params, batches, self._state_now())
+        batches = held[4]
         if len(batches) != 1 or len(batches[0].params) != len(params):
             grads = [list(map(_grad, batch.params)) for batch in batches]
         else:
