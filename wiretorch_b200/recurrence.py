@@ -179,12 +179,9 @@ def gated_scan(a, x, state=None, *, form="decay", starts=None, lengths=None):
             raise ValueError(f"state must be float32 of shape {(B, N)} on {x.device}")
         starts = _per_trial("starts", starts, (B, T), (torch.bool,), x)
         lengths = _per_trial("lengths", lengths, (B,), (torch.int32, torch.int64), x)
-    if starts is not None:
-        starts = starts.contiguous()
-    if lengths is not None:
-        lengths = (lengths if lengths.dtype == torch.int32 else lengths.clamp(0, T).int()).contiguous()
-    if state is not None:
-        state = state.contiguous()
+        starts, state = (t if t is None else t.contiguous() for t in (starts, state))
+        if lengths is not None:
+            lengths = (lengths if lengths.dtype == torch.int32 else lengths.clamp(0, T).int()).contiguous()
     want = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (a, x, state))
     return _GatedScan.apply(a, x, state, starts, lengths, code, want)
 
