@@ -15,3 +15,35 @@ def test_dimensions_are_refused_whatever_comes_with_them():
                    {"starts": torch.zeros(shape[:2], dtype=torch.bool, device="cuda")}):  # fmt: skip
             with pytest.raises(ValueError, match="dimensions"):
                 recurrence.gated_scan(x, x, **kw)
+
+
+@pytest.mark.parametrize("which", ["scalar", "1", "B11", "N", "every other"])
+def test_a_broadcast_decay_is_not_written_out(which):
+    """A call with a decay that is one value, one a trial or one a neuron takes no memory beyond its results
+    (and keeps none beside x and h for the backward pass), a decay read with a stride that of its own size."""
+    B, T, N = 8, 50, 20_000
+    x = torch.rand((B, T, N), device="cuda")
+    a = torch.rand({"scalar": (), "1": (1,), "B11": (B, 1, 1), "N": (N,), "every other": (2 * N,)}[which], device="cuda")
+    a = (a[::2] if which == "every other" else a).requires_grad_(True)
+    size, rows = 4 * B * T * N, 4 * B * N
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    h, last = recurrence.gated_scan(a, x)
+    assert torch.cuda.max_memory_allocated() - before <= size + 4 * rows + (1 << 21)
+    want, end = recurrence.gated_scan(a.detach().expand(B, T, N).contiguous(), x)
+    assert torch.equal(h, want) and torch.equal(last, end)
+    (da,) = torch.autograd.grad(last.sum(), a)
+    assert da.shape == a.shape and bool(torch.isfinite(da).all())
+    state = torch.zeros((B, N), device="cuda")
+    step = recurrence.gated_step(a.detach().expand(B, 1, N)[:, 0] if which == "B11" else a.detach(), x[:, 0], state)
+    assert torch.equal(step, h[:, 0].detach())
+
+
+def test_decays_that_do_not_expand_are_refused():
+    x = torch.zeros((2, 3, 4), device="cuda")
+    for shape in ((5,), (3, 3, 1), (2, 2, 4), (1, 2, 3, 4), (2, 3, 0)):
+        with pytest.raises(ValueError, match="expand"):
+            recurrence.gated_scan(torch.zeros(shape, device="cuda"), x)
+    with pytest.raises(ValueError, match="expand"):  # x smaller than a
+        recurrence.gated_scan(torch.zeros((2, 3, 4), device="cuda"), x[..., :1])

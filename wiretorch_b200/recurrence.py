@@ -70,11 +70,13 @@ def _checked(a, x, dims):
         raise TypeError(f"the recurrence takes float32, bfloat16 and float16, not {x.dtype}")
     if a.dtype != x.dtype or a.device != x.device:
         raise TypeError(f"a and x must have one type and device: {a.dtype} on {a.device}, {x.dtype} on {x.device}")
-    try:
-        a = a if a.shape == x.shape else a.expand(x.shape)
+    if a.shape == x.shape:
+        return _unit(a), _unit(x)
+    try:  # rows are written out before they are broadcast over trials and time
+        row = _unit(a.expand(*a.shape[:-1], x.shape[-1]))
+        return row.expand(x.shape), _unit(x)
     except RuntimeError:
         raise ValueError(f"a of shape {tuple(a.shape)} does not expand to x's {tuple(x.shape)}") from None
-    return _unit(a), _unit(x)
 
 
 def _unit(t):
