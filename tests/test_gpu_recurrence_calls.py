@@ -47,3 +47,22 @@ def test_decays_that_do_not_expand_are_refused():
             recurrence.gated_scan(torch.zeros(shape, device="cuda"), x)
     with pytest.raises(ValueError, match="expand"):  # x smaller than a
         recurrence.gated_scan(torch.zeros((2, 3, 4), device="cuda"), x[..., :1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("form", ["decay", "sigmoid"])
+def test_h_may_be_changed_in_place_where_the_backward_pass_does_not_read_it(dtype, form):
+    """Chunks of at most 8 steps, and 16-bit ones of any length."""
+    for T in (1, 5, 8, 9, 200):
+        a, x = (torch.rand((3, T, 10), device="cuda").to(dtype).requires_grad_(True) for _ in range(2))
+        state = torch.rand((3, 10), device="cuda", requires_grad=True)
+        grads = []
+        for change in (False, True):
+            h, last = recurrence.gated_scan(a, x, state, form=form)
+            out = (h.mul_(0.5) if change else h * 0.5).float().sum() + last.sum()
+            if change and T > 8 and dtype == torch.float32:
+                with pytest.raises(RuntimeError, match="inplace operation"):
+                    torch.autograd.grad(out, [a, x, state])
+            else:
+                grads.append(torch.autograd.grad(out, [a, x, state]))
+        assert all(torch.equal(p, q) for p, q in zip(grads[0], grads[-1]))

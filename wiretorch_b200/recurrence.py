@@ -118,7 +118,8 @@ class _GatedScan(torch.autograd.Function):
             _lib.check(rc, "wt_gated_scan")
         _lib.count_launches(1)
         if want_grad:
-            ctx.save_for_backward(a, x, state, starts, lengths, work if saves else h)
+            # a chunk of one segment needs neither h nor saved states
+            ctx.save_for_backward(a, x, state, starts, lengths, work if saves else h if T > SEGMENT else None)
             ctx.form, ctx.given, ctx.from_h = form, given, not saves
         return h, last
 
@@ -141,7 +142,7 @@ class _GatedScan(torch.autograd.Function):
         dstate = torch.empty_like(dlast) if ctx.needs_input_grad[2] else None
         size = lib.wt_gated_scratch_bytes(B, T, N, kind, 1)
         scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-        h, saved = (kept.data_ptr(), None) if ctx.from_h else (None, kept.data_ptr())
+        h, saved = (_at(kept), None) if ctx.from_h else (None, _at(kept))
         s = _Grad(B, T, N, kind, ctx.form, reduce, TYPES[da.dtype],
                   a.data_ptr(), a.stride(0), 0 if reduce else a.stride(1), x.data_ptr(), x.stride(0), x.stride(1),
                   _at(state), _at(starts), _at(lengths), h, saved, dh.data_ptr(), dh.stride(0), dh.stride(1),
