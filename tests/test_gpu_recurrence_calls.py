@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from wiretorch_b200 import recurrence
+from wiretorch_b200 import _lib, recurrence
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +66,10 @@ def test_h_may_be_changed_in_place_where_the_backward_pass_does_not_read_it(dtyp
             else:
                 grads.append(torch.autograd.grad(out, [a, x, state]))
         assert all(torch.equal(p, q) for p, q in zip(grads[0], grads[-1]))
+
+
+def test_the_current_stream_of_a_device_by_every_name():
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for device in (0, None, "cuda", "cuda:0", torch.device("cuda"), torch.device("cuda", 0), side.device):
+            assert _lib.stream_of(device) == side.cuda_stream

@@ -1,9 +1,9 @@
-"""Refusals of the gated recurrence that need no GPU."""
+"""Refusals on the way to the kernels that need no GPU."""
 
 import pytest
 import torch
 
-from wiretorch_b200 import recurrence
+from wiretorch_b200 import _lib, recurrence
 
 
 def test_what_is_not_three_dimensional_is_refused_whatever_comes_with_it():
@@ -13,3 +13,9 @@ def test_what_is_not_three_dimensional_is_refused_whatever_comes_with_it():
     for kw in more:
         with pytest.raises(RuntimeError, match="CUDA tensors only"):
             recurrence.gated_scan(x, x, **kw)
+
+
+def test_a_device_that_is_not_a_gpu_has_no_stream():
+    for device in ("cpu", torch.device("cpu"), torch.device("cpu", 0), "meta"):
+        with pytest.raises(ValueError, match="no CUDA stream"):
+            _lib.stream_of(device)

@@ -176,9 +176,11 @@ def stream_of(device) -> int:
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
             lambda index: torch.cuda.current_stream(index).cuda_stream)  # fmt: skip
     index = device if isinstance(device, int) else getattr(device, "index", None)
-    if index is None or callable(index):  # no index, or a name
+    if not isinstance(index, int) or getattr(device, "type", "cuda") != "cuda":  # no index, a name, or no GPU's
         import torch
 
-        index = torch.device(device).index
-        index = torch.cuda.current_device() if index is None else index
+        named = torch.device("cuda" if device is None else device)
+        if named.type != "cuda":
+            raise ValueError(f"{named} has no CUDA stream")
+        index = torch.cuda.current_device() if named.index is None else named.index
     return _raw_stream(index)
