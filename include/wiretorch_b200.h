@@ -582,7 +582,8 @@ int wt_adamw_step(const WtAdamW *a, void *stream);
  *   WT_GATED_DECAY:   h_t = a_t h_{t-1} + x_t
  *   WT_GATED_SIGMOID: f_t = 1 / (1 + exp(-a_t)), h_t = f_t h_{t-1} + (1 - f_t) x_t
  * a, x and h are of `type`, the state float. Strides are in elements; the last dimension has
- * unit stride, and a stride of 0 over trials or time is a broadcast. */
+ * unit stride, and a stride of 0 over trials or time is a broadcast. At most 2^31 - 256 trials or
+ * columns and 2^30 steps. */
 #define WT_GATED_DECAY 0
 #define WT_GATED_SIGMOID 1
 #define WT_GATED_SEGMENT 8 /* steps between saved states */

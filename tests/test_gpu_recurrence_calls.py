@@ -73,3 +73,15 @@ def test_the_current_stream_of_a_device_by_every_name():
     with torch.cuda.stream(side):
         for device in (0, None, "cuda", "cuda:0", torch.device("cuda"), torch.device("cuda", 0), side.device):
             assert _lib.stream_of(device) == side.cuda_stream
+
+
+def test_sizes_past_the_kernels_numbers_are_refused():
+    """Sizes that 32 bits would cut: broadcast inputs, so that nothing of the size is ever held."""
+    one = torch.zeros((1, 1, 1), device="cuda")
+    for shape in ((2**32 + 8, 1, 1), (1, 1, 2**32 + 8), (2**31 - 255, 1, 1), (1, 1, 2**31 - 255), (1, 2**30 + 1, 1)):
+        with pytest.raises(ValueError, match="at most"):
+            recurrence.gated_scan(one[0, 0, 0], one.expand(shape))
+        if shape[1] == 1:
+            x = one.expand(shape)[:, 0]
+            with pytest.raises(ValueError, match="at most"):
+                recurrence.gated_step(one[0, 0, 0], x, x)

@@ -364,7 +364,8 @@ int wt_adamw_step(const WtAdamW *a, void *stream) {
 }
 
 static bool bad_gated(int B, int T, int N, int type, int form) {
-    return B < 0 || T < 0 || T > (1 << 30) || N < 0 || type < WT_F32 || type > WT_F16 || form < WT_GATED_DECAY || form > WT_GATED_SIGMOID;
+    constexpr int kMost = INT32_MAX - 255;  // the kernels round columns up to whole warps' in 32 bits
+    return B < 0 || B > kMost || T < 0 || T > (1 << 30) || N < 0 || N > kMost || type < WT_F32 || type > WT_F16 || form < WT_GATED_DECAY || form > WT_GATED_SIGMOID;
 }
 
 int32_t wt_gated_parts(int32_t B, int32_t T, int32_t N, int32_t type, int32_t backward) {

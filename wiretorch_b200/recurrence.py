@@ -22,6 +22,7 @@ _C = _lib.C
 SEGMENT = 8  # WT_GATED_SEGMENT: steps between the states saved for the backward pass
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # WT_F32, WT_BF16, WT_F16
 FORMS = {"decay": 0, "sigmoid": 1}
+MOST, MOST_STEPS = (1 << 31) - 256, 1 << 30  # trials or columns, and steps, of a call
 
 
 class _Scan(_C.Structure):
@@ -70,6 +71,8 @@ def _checked(a, x, dims):
         raise TypeError(f"the recurrence takes float32, bfloat16 and float16, not {x.dtype}")
     if a.dtype != x.dtype or a.device != x.device:
         raise TypeError(f"a and x must have one type and device: {a.dtype} on {a.device}, {x.dtype} on {x.device}")
+    if max(x.shape) > MOST or (dims == 3 and x.shape[1] > MOST_STEPS):
+        raise ValueError(f"a call takes at most {MOST} trials or columns and {MOST_STEPS} steps, not {tuple(x.shape)}")
     if a.shape == x.shape:
         return _unit(a), _unit(x)
     try:  # rows are written out before they are broadcast over trials and time
