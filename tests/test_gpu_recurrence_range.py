@@ -135,3 +135,17 @@ def test_infinities_stay_where_products_of_decays_underflow(B, T, N, form, value
     assert torch.isinf(rh[..., :4]).any(1).all() and torch.isinf(rdx[..., 4:6]).any(1).all()
     for name, got, want in (("h", h, rh), ("last", last, rlast), ("dx", dx, rdx), ("dstate", dstate, rdstate)):
         assert torch.allclose(got, want, rtol=0.0, atol=32 * U, equal_nan=True), name
+
+
+@pytest.mark.parametrize("form,cuts", [("decay", True), ("sigmoid", False)])
+def test_as_many_parts_as_there_can_be(form, cuts):
+    """2,048 parts of 16 steps, against the definition with the tolerances of the gated recurrence's tests."""
+    import test_gpu_recurrence as general
+
+    B, T, N = 1, 32_768, 4
+    assert parts(B, T, N, torch.float32, 0) == parts(B, T, N, torch.float32, 1) == 2048
+    a, x, state, dh, dlast = general.inputs(B, T, N, form, torch.float32, 3)
+    starts = None
+    if cuts:
+        starts = torch.rand((B, T), device="cuda", generator=torch.Generator("cuda").manual_seed(2)) < 2e-4
+    general.check(a, x, state, dh, dlast, form, starts=starts)
