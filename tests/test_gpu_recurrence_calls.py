@@ -78,6 +78,8 @@ def test_the_current_stream_of_a_device_by_every_name():
 def test_sizes_past_the_kernels_numbers_are_refused():
     """Sizes that 32 bits would cut: broadcast inputs, so that nothing of the size is ever held."""
     one = torch.zeros((1, 1, 1), device="cuda")
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
     for shape in ((2**32 + 8, 1, 1), (1, 1, 2**32 + 8), (2**31 - 255, 1, 1), (1, 1, 2**31 - 255), (1, 2**30 + 1, 1)):
         with pytest.raises(ValueError, match="at most"):
             recurrence.gated_scan(one[0, 0, 0], one.expand(shape))
@@ -85,3 +87,4 @@ def test_sizes_past_the_kernels_numbers_are_refused():
             x = one.expand(shape)[:, 0]
             with pytest.raises(ValueError, match="at most"):
                 recurrence.gated_step(one[0, 0, 0], x, x)
+    assert torch.cuda.max_memory_allocated() == before

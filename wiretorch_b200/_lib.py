@@ -175,7 +175,9 @@ def stream_of(device) -> int:
         # the handle without a Stream object around it (2 us a call); the long way without it
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
             lambda index: torch.cuda.current_stream(index).cuda_stream)  # fmt: skip
-    index = device if isinstance(device, int) else getattr(device, "index", None)
+    if type(device) is int:
+        return _raw_stream(device)
+    index = getattr(device, "index", None)
     if not isinstance(index, int) or getattr(device, "type", "cuda") != "cuda":  # no index, a name, or no GPU's
         import torch
 

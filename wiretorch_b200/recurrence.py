@@ -71,8 +71,6 @@ def _checked(a, x, dims):
         raise TypeError(f"the recurrence takes float32, bfloat16 and float16, not {x.dtype}")
     if a.dtype != x.dtype or a.device != x.device:
         raise TypeError(f"a and x must have one type and device: {a.dtype} on {a.device}, {x.dtype} on {x.device}")
-    if max(x.shape) > MOST or (dims == 3 and x.shape[1] > MOST_STEPS):
-        raise ValueError(f"a call takes at most {MOST} trials or columns and {MOST_STEPS} steps, not {tuple(x.shape)}")
     if a.shape == x.shape:
         return _unit(a), _unit(x)
     try:  # rows are written out before they are broadcast over trials and time
@@ -84,6 +82,10 @@ def _checked(a, x, dims):
 
 def _unit(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _too_large(x):
+    return ValueError(f"a call takes at most {MOST} trials or columns and {MOST_STEPS} steps, not {tuple(x.shape)}")
 
 
 def _per_trial(name, t, shape, dtypes, x):
@@ -181,11 +183,16 @@ def gated_scan(a, x, state=None, *, form="decay", starts=None, lengths=None):
             return gated_scan(a, x, state, form=form, starts=starts, lengths=lengths)
     if x.dim() == 3:
         B, T, N = x.shape
+        if B > MOST or N > MOST or T > MOST_STEPS:
+            raise _too_large(x)
         if state is not None and (state.dtype != torch.float32 or state.device != x.device or tuple(state.shape) != (B, N)):
             raise ValueError(f"state must be float32 of shape {(B, N)} on {x.device}")
         starts = _per_trial("starts", starts, (B, T), (torch.bool,), x)
         lengths = _per_trial("lengths", lengths, (B,), (torch.int32, torch.int64), x)
-        starts, state = (t if t is None else t.contiguous() for t in (starts, state))
+        if state is not None:
+            state = state.contiguous()
+        if starts is not None:
+            starts = starts.contiguous()
         if lengths is not None:
             lengths = (lengths if lengths.dtype == torch.int32 else lengths.clamp(0, T).int()).contiguous()
     want = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (a, x, state))
@@ -201,11 +208,14 @@ def gated_step(a, x, state, *, form="decay"):
             return gated_step(a, x, state, form=form)
     if torch.is_grad_enabled() and (a.requires_grad or x.requires_grad or state.requires_grad):
         raise RuntimeError("gated_step has no gradient: use gated_scan, or call it under torch.no_grad()")
+    if x.dim() == 2:
+        B, N = x.shape
+        if B > MOST or N > MOST:
+            raise _too_large(x)
     a, x = _checked(a, x, 2)
     if state.dtype != torch.float32 or state.shape != x.shape or state.device != x.device or not state.is_contiguous():
         raise ValueError(f"state must be contiguous float32 of shape {tuple(x.shape)} on {x.device}")
     h = torch.empty_like(x, memory_format=torch.contiguous_format)
-    B, N = x.shape
     s = _Step(B, N, TYPES[x.dtype], code, a.data_ptr(), a.stride(0), x.data_ptr(), x.stride(0), state.data_ptr(), h.data_ptr())
     with _lib.timed("wt_gated_step"):
         rc = _lib.lib().wt_gated_step(_C.byref(s), _C.c_void_p(_lib.stream_of(x.get_device())))
