@@ -524,7 +524,8 @@ int wt_pack_spikes(const WtSpikeBits *a, void *stream);
  * left out; zeroed by the caller once, then kept. */
 typedef struct {
     float norm, clip;   /* the last norm, and min(1, max_norm / (norm + 1e-6)) */
-    int32_t skip;       /* the last norm was not finite: the step is left out */
+    int32_t skip;       /* the last norm was not finite (squares are float's: 1.8e19 is the most
+                         * a gradient may be): the step is left out */
     uint32_t arrived;
     int64_t skipped;    /* steps left out so far */
 } WtStepControl;
@@ -551,8 +552,8 @@ int wt_grad_norm(const WtGradNorm *a, void *stream);
 
 /* One AdamW step of n tensors of one type (host arrays, read before the call returns; the
  * addresses are the device's). state_bits 32: m and v float; 8: m and v e4m3 codes with one
- * float scale per WT_ADAMW_BLOCK elements, rounded by random bits hashed from (seed, count,
- * the element's number: first[k] + its place). 16-bit tensors have a float master, which is
+ * float scale per WT_ADAMW_BLOCK elements, rounded by random bits hashed from the low 32 bits of
+ * seed and count and the element's number, first[k] + its place. 16-bit tensors have a float master, which is
  * stepped, and the tensor written as its rounding. With `control` (of a wt_grad_norm before
  * it on the stream) the gradients are scaled by its clip and the step is left out when its norm
  * was not finite. The step number of the bias corrections is step - *skipped, the steps left out so

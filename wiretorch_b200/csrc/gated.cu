@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(block_of(WIDE)) maps_kernel(const Args s, cons
 // Joins the maps of a trial's parts into the states that enter them: a block takes COLS columns,
 // each of the 32 / COLS x WARPS threads of a column a run of up to RUN parts, held in registers.
 // Runs are joined within a warp by shuffles, then over the warps. Latency: 37 parts of 8,192
-// columns 6 us, 1,640 parts of 64 columns 9.5.
+// columns 6 us, 2,048 parts of 64 columns 10.
 template <bool FORWARD, bool CUTS, int COLS, int WARPS, int RUN>
 __global__ void __launch_bounds__(32 * WARPS) join_kernel(const Maps maps, const float *state, int N) {
     constexpr int kIn = 32 / COLS, kRuns = kIn * WARPS;

@@ -176,7 +176,8 @@ def gated_scan(a, x, state=None, *, form="decay", starts=None, lengths=None):
     Gradients flow to ``a``, ``x`` and ``state`` (detach it between chunks to truncate), first
     ones only; the state and the sums are float32, each result rounded once. Decays of size up to
     about 1 are what it is for: where some are larger, the product of the decays over any stretch
-    of time has to stay in float32's range, or the state that enters the stretch has to be 0."""
+    of time has to stay in float32's range, or the state that enters the stretch has to be 0. An
+    infinite decay gives an infinity or NaN."""
     code = _form(form)
     if x.is_cuda and x.get_device() != torch.cuda.current_device():
         with torch.cuda.device(x.get_device()):
